@@ -144,7 +144,6 @@ __global__ __launch_bounds__(64 * kWaves, row_waves(D, sizeof(T) == 4) / kWaves)
         const int last_n = row_last(a, rq, i_row), first_n = row_first(a, rq, i_row);
         // keys every row of the tile sees
         const int all_first = row_first(a, rq, i_last), all_last = row_last(a, rq, i_first);
-        const int any_first = row_first(a, rq, i_first);
 
         // The pages of a step's first and last 16 tokens; past the last step those of the last. A wave looks up those of
         // its next 64 steps at once, a lane each (one lookup a step would keep every step's LDS reads waiting for it:
@@ -288,9 +287,10 @@ __global__ __launch_bounds__(64 * kWaves, row_waves(D, sizeof(T) == 4) / kWaves)
         // score is 3 above it, and at the row's first: a row's largest scores come early, and moving costs as many
         // products as the row has elements.
         float base = 0.0f, l = 0.0f, limit = -INFINITY;
-        // Exponent field of the largest value scale so far: the products of probabilities (up to 8) and scales are
-        // scaled by 2^(25 - top), to below 2^14.
-        int top = 1;
+        // Exponent field of the largest value scale that the row has seen: the products of its probabilities (up to 8) and
+        // scales are scaled by 2^(25 - top), to below 2^14. Each row has its own: by a token that it does not see, its
+        // products could fall below what fp16 holds.
+        int top = 1, least_top = 1;  // least_top: of the tile's rows
         float up = 0x1p24f;
 
         auto multiply = [&](int step, Pages pages, const uint8_t *stage, auto refill) __attribute__((always_inline)) {
@@ -355,32 +355,33 @@ __global__ __launch_bounds__(64 * kWaves, row_waves(D, sizeof(T) == 4) / kWaves)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] -= by;
             }
-            // the largest value scale of the step's visible tokens
+            // whether a value scale of the step may be larger than a row has seen
             int largest = 0;
 #pragma unroll
             for (int i = 0; i < (NB + 3) / 4; ++i) {
                 const uint32_t two = values.top[i] & 0x7fff7fffu;
                 largest = max(largest, int(max(two & 0xffffu, two >> 16)));
             }
-            if (__any(largest >= (top + 1) << 10)) {
-                largest = 0;
+            if (__any(largest >= (least_top + 1) << 10)) {
+                // of what this row sees (hidden tokens' scales are 0 here); one that is not finite becomes negative and
+                // does not count
+                typedef short s16x8 __attribute__((ext_vector_type(8)));
+                s16x8 most = {};
 #pragma unroll
-                for (int i = 0; i < (NB + 3) / 4; ++i)
+                for (int i = 0; i < NB; ++i)
+                    most = __builtin_elementwise_max(most, (__builtin_bit_cast(s16x8, values.scale[i]) & (short)0x7fff) + (short)0x0400);
+                int seen = 0;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int field = values.top[i] >> (10 + 16 * e) & 31;
-                        const int key = key0 + 8 * g + (2 * (n % (4 * NB)) + e + 32 * i) / NB;
-                        if (page_ok && key >= any_first && key < key_hi && field < 31) largest = max(largest, field);
-                    }
+                for (int i = 0; i < 8; ++i) seen = max(seen, (int)most[i]);
+                seen = max(top, (seen >> 10) - 1);
+                seen = max(seen, xor_shfl<16>(seen));
+                seen = max(seen, xor_shfl<32>(seen));
+                const float down = ldexpf(1.0f, top - seen);
 #pragma unroll
-                for (int w = 1; w < 64; w <<= 1) largest = max(largest, __shfl_xor(largest, w, 64));
-                if (largest > top) {
-                    const float down = ldexpf(1.0f, top - largest);
-#pragma unroll
-                    for (int t = 0; t < kTiles; ++t) o[t] *= down;
-                    top = largest;
-                    up = ldexpf(1.0f, 25 - top);
-                }
+                for (int t = 0; t < kTiles; ++t) o[t] *= down;
+                top = seen;
+                up = ldexpf(1.0f, 25 - top);
+                least_top = butterfly<8>(top, [](int x, int y) { return min(x, y); });
             }
 
             float p[8];
