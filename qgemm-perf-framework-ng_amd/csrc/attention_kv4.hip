@@ -285,7 +285,8 @@ __global__ __launch_bounds__(64 * kWaves, row_waves(D, sizeof(T) == 4) / kWaves)
         f32x4 o[kTiles] = {};
         // Probabilities are 2^(score - base) with a whole number for base, so that moving it is exact. It moves when a
         // score is 3 above it, and at the row's first: a row's largest scores come early, and moving costs as many
-        // products as the row has elements.
+        // products as the row has elements. (Past 2^24 the base itself is rounded, to what fp32 tells apart of the
+        // scores; what it moves by is not, so that the row's largest probability is 1 all the same.)
         float base = 0.0f, l = 0.0f, limit = -INFINITY;
         // Exponent field of the largest value scale that the row has seen: the products of its probabilities (up to 8) and
         // scales are scaled by 2^(25 - top), to below 2^14. Each row has its own: by a token that it does not see, its
@@ -345,7 +346,7 @@ __global__ __launch_bounds__(64 * kWaves, row_waves(D, sizeof(T) == 4) / kWaves)
                 mx = __builtin_elementwise_maximum(mx, xor_shfl<16>(mx));
                 mx = __builtin_elementwise_maximum(mx, xor_shfl<32>(mx));
                 const bool first = limit == -INFINITY;
-                const float by = mx > (first ? -INFINITY : 0.0f) ? rintf(base + mx) - base : 0.0f;
+                const float by = mx > (first ? -INFINITY : 0.0f) ? rintf(mx) : 0.0f;
                 if (mx > -INFINITY) limit = 3.0f;
                 const float alpha = first ? 1.0f : exp2_of(-by);
                 base += by;

@@ -477,7 +477,9 @@ __global__ __launch_bounds__(64 * W, 1) void attention_kv4_prompt_kernel(AttendA
             }
             // The base is taken so that the largest probability is 2^12, and moves to a larger score only once that
             // is 3 above: up to 2^15 fp16 still holds them, and a row's largest scores come early. A tile with values
-            // divided by 8 uses those 3 itself and moves at once.
+            // divided by 8 uses those 3 itself and moves at once. (Past 2^24 the base itself is rounded, to what fp32
+            // tells apart of the scores. Past 2^26 x - 12 is x - 16, then x: the largest probability is cut to what fp16
+            // holds, or is 1.)
             float mx[2];
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
@@ -496,7 +498,7 @@ __global__ __launch_bounds__(64 * W, 1) void attention_kv4_prompt_kernel(AttendA
                     x = __builtin_elementwise_maximum(x, xor_shfl<16>(x));
                     x = __builtin_elementwise_maximum(x, xor_shfl<32>(x));
                     const bool first = limit[w] == -INFINITY;
-                    const float by = x > (first ? -INFINITY : 12.0f) ? rintf(base[w] + (x - 12.0f)) - base[w] : 0.0f;
+                    const float by = x > (first ? -INFINITY : 12.0f) ? rintf(x - 12.0f) : 0.0f;
                     if (x > -INFINITY) limit[w] = 15.0f;
                     const float alpha = first ? 1.0f : exp2_of(-by);
                     base[w] += by;
@@ -504,7 +506,9 @@ __global__ __launch_bounds__(64 * W, 1) void attention_kv4_prompt_kernel(AttendA
 #pragma unroll
                     for (int t = 0; t < kDepth; ++t) o[w][t] *= alpha;
 #pragma unroll
-                    for (int t = 0; t < kPass; ++t) s[w][t] -= by;
+                    for (int t = 0; t < kPass; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[w][t][i] = __builtin_elementwise_minimum(s[w][t][i] - by, most + 0.5f);
                     if (!kRaw && plain) minus_base[w] = f32x4{-base[w], -base[w], -base[w], -base[w]};
                 }
             }
