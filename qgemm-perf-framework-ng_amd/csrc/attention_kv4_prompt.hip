@@ -33,12 +33,13 @@
 // probabilities and fp32 queries to 22 bits in the same way: three products in
 // the place of one.
 //
-// Scales of 2^13 and more (values past 65504) would overflow: a wave that finds one
-// among the tokens it decodes divides all of theirs by 8, and says so beside the
-// tile; their scores are multiplied by 8 within the exponent's product, their
-// probabilities by 3 more in the exponent. Values whose scale is not finite are
-// decoded as 0, and the rows that see them are set to NaN at the end. These, and
-// pages outside the cache, mark the tile: only marked tiles look for them.
+// Scales of 2^13 and more (values past 65504) would overflow: a token with one is
+// decoded divided by 8, and alone (small scales would lose bits, and rows that do
+// not see that token must not lose theirs). Its scores are multiplied by 8 within
+// the exponent's product, its probabilities by 3 more in the exponent. Values whose
+// scale is not finite are decoded as 0, and the rows that see them are set to NaN at
+// the end. These, and pages outside the cache, mark the tile: only marked tiles look
+// for them.
 #include "attention_common.h"
 
 namespace pfng {
@@ -57,7 +58,6 @@ struct PromptShape {
     static constexpr int kBuffer = 2 * kParts * kPart;                // keys, then values
     static constexpr int kPieces = KT * kRowPieces / (32 * W);        // of 16 bytes, a thread's
     static constexpr int kRowLanes = 64 / kRowPieces;                 // tokens of 64 key pieces
-    static constexpr int kGroups = KT / 8;                            // of 8 tokens
     static_assert(kPieces >= 1 && kPieces * 32 * W == KT * kRowPieces && KT * D / 512 * 16 == KT * kRowPieces,
                   "whole pieces");
 };
@@ -89,9 +89,9 @@ __global__ __launch_bounds__(64 * W, 1) void attention_kv4_prompt_kernel(AttendA
     constexpr int kPass = S::kExact || D == 256 ? 2 : 4;
     extern __shared__ __align__(16) uint8_t lds[];  // two buffers
     __shared__ int marked[2];                       // the step that last marked each buffer
-    // of each 8 tokens: what scores are multiplied by, and what is added to the probabilities' exponents;
-    // [half of a tile of 16][tile], as lane group g meets them (its half is g / 2)
-    __shared__ __align__(16) float key_factor[2][2][S::kGroups / 2], value_shift[2][2][S::kGroups / 2];
+    // of each token: what multiple of a score is added to it (0, or 7 of a divided one), and what to the exponents of the
+    // probabilities
+    __shared__ __align__(16) float score_more[2][KT], value_shift[2][KT];
 
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -280,34 +280,34 @@ __global__ __launch_bounds__(64 * W, 1) void attention_kv4_prompt_kernel(AttendA
             uint8_t *buffer = lds + (step & 1) * S::kBuffer;
             const int my_token = token_of(u);
             constexpr int kKeyScales = NB == 2 ? 1 : 2;
-            bool big = false;
+            uint32_t big = 0;  // bit t: the piece's token t is divided by 8 (keys: a piece is of one token)
             // of keys not before here: looked at where the tile is loaded, it would be waited for there
             const uint32_t check = !keys ? in.check : NB > 2 && (piece / (NB > 2 ? NB / 4 : 1)) & 1 ? in.scale[1] : in.scale[0];
             if (__any(!in.page_ok || large_scale(check))) {
                 const int scales = keys ? 2 * kKeyScales : 16;
+                auto token_at = [&](int i) { return keys ? 0 : i / NB; };
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (i < scales) {
                         const int e = exponent_of(in.scale[i / 2] >> (16 * (i & 1)));
-                        big |= e >= 28 && e < 31;
+                        big |= uint32_t(e >= 28 && e < 31) << token_at(i);
                     }
-                big = __any(big);
+                if constexpr (NB == 8)  // the scales of a key are between two lanes
+                    if (keys) big |= (uint32_t)xor_shfl<S::kRowLanes>((int)big);
                 if (lane == 0) marked[step & 1] = step;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (i < scales) {
                         f16x2 two = __builtin_bit_cast(f16x2, in.scale[i / 2]);
-                        if (big) two[i & 1] = two[i & 1] * (_Float16)0.125f;
+                        if (big >> token_at(i) & 1) two[i & 1] = two[i & 1] * (_Float16)0.125f;
                         if (!keys && exponent_of(in.scale[i / 2] >> (16 * (i & 1))) == 31) two[i & 1] = (_Float16)0.0f;
                         in.scale[i / 2] = __builtin_bit_cast(uint32_t, two);
                     }
             }
-            // the groups of 8 tokens of this piece: 8, 16 or 32 tokens
-            constexpr int kPieceGroups = S::kRowLanes / 8;
-            if (lane < kPieceGroups) {
-                const int g8 = (decoder * S::kPieces + u) * kPieceGroups + lane;
-                if (keys) key_factor[step & 1][g8 & 1][g8 >> 1] = big ? 8.0f : 1.0f;
-                else value_shift[step & 1][g8 & 1][g8 >> 1] = big ? 3.0f : 0.0f;
+            if (keys) {
+                if (lane < S::kRowLanes) score_more[step & 1][my_token] = big ? 7.0f : 0.0f;
+            } else {
+                if (c < S::kChunkTokens) value_shift[step & 1][my_token + c] = big >> c & 1 ? 3.0f : 0.0f;
             }
             if (keys) {
 #pragma unroll
@@ -365,9 +365,6 @@ __global__ __launch_bounds__(64 * W, 1) void attention_kv4_prompt_kernel(AttendA
         float base[2] = {0.0f, 0.0f}, l[2] = {0.0f, 0.0f};
         float limit[2] = {-INFINITY, -INFINITY};  // base moves when an exponent is above: at the first one, then at 15
         f32x4 minus_base[2] = {};
-        float share[kPass];  // of a probability in the sum, by tile of 16 keys: 1, or 1/8 where it is times 8
-#pragma unroll
-        for (int t = 0; t < kPass; ++t) share[t] = 1.0f;
         uint32_t broken[2] = {0, 0};  // blocks of the row that are NaN
 
         // of a marked tile's token: bit 0 no page, bit 1 + b block b of its values is NaN
@@ -394,7 +391,8 @@ __global__ __launch_bounds__(64 * W, 1) void attention_kv4_prompt_kernel(AttendA
             const uint8_t *key_operands = lds + (step & 1) * S::kBuffer + t0 * NB * 1024 + lane * 16;
             const uint8_t *value_operands =
                 lds + (step & 1) * S::kBuffer + S::kParts * S::kPart + t0 / 2 * kDepth * 1024 + lane * 16;
-            const float *factors = &key_factor[step & 1][g >> 1][t0], *shifts = &value_shift[step & 1][g >> 1][t0];
+            // of tile t's keys that this lane has: at 16 t
+            const float *more = &score_more[step & 1][16 * t0 + 4 * g], *shifts = &value_shift[step & 1][16 * t0 + 4 * g];
             const int key0 = key_lo + step * KT + 16 * t0;
             if (key0 >= any_last || key0 + 16 * kPass <= any_first) return;
             const bool whole = key0 >= all_first && key0 + 16 * kPass <= all_last;
@@ -438,19 +436,28 @@ __global__ __launch_bounds__(64 * W, 1) void attention_kv4_prompt_kernel(AttendA
 #pragma unroll
             for (int r = 0; r < kAhead; ++r) ring[r] = read_values(r);
             auto key_of = [&](int t, int i) { return key0 + 16 * t + 4 * g + i; };
-            if (kRaw || odd || !plain) {
+            if (odd) {
+                // of what the scores are without the base
 #pragma unroll
                 for (int t = 0; t < kPass; ++t) {
-                    const float f = odd ? factors[t] : 1.0f;
+                    const f32x4 times = *reinterpret_cast<const f32x4 *>(more + 16 * t);
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const float within = kRaw || !plain ? 0.0f : base[w];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            s[w][t][i] = __builtin_fmaf(s[w][t][i] + within, times[i], s[w][t][i]);
+                    }
+                    pin_order();
+                }
+            }
+            if (kRaw || !plain) {
+#pragma unroll
+                for (int t = 0; t < kPass; ++t)
 #pragma unroll
                     for (int w = 0; w < 2; ++w)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float x = s[w][t][i];
-                            if (kRaw || !plain) s[w][t][i] = __builtin_fmaf(x, back[w] * f, -base[w]);
-                            else if (f != 1.0f) s[w][t][i] = __builtin_fmaf(x + base[w], f, -base[w]);
-                        }
-                }
+                        for (int i = 0; i < 4; ++i) s[w][t][i] = __builtin_fmaf(s[w][t][i], back[w], -base[w]);
             }
             if (!whole || odd) {
                 uint32_t hidden = 0;  // one bit for each of the lane's keys
@@ -513,12 +520,19 @@ __global__ __launch_bounds__(64 * W, 1) void attention_kv4_prompt_kernel(AttendA
                 }
             }
             if (odd) {
+                // probabilities of divided values are 8 times as large, and enter the sum as they are: 7/8 of them leave it
 #pragma unroll
                 for (int t = 0; t < kPass; ++t) {
-                    const float shift = shifts[t];
-                    s[0][t] += shift;
-                    s[1][t] += shift;
-                    share[t] = shift != 0.0f ? 0.125f : 1.0f;
+                    const f32x4 shift = *reinterpret_cast<const f32x4 *>(shifts + 16 * t);
+#pragma unroll
+                    for (int w = 0; w < 2; ++w)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (shift[i] != 0.0f) {
+                                const float p = exp2_of(s[w][t][i] += shift[i]);
+                                l[w] -= 0.875f * (S::kParts == 1 ? (float)(_Float16)p : p);
+                            }
+                    pin_order();
                 }
             }
             // Probabilities of 8 keys a lane at a time, of two tiles; the next ones between the products with these.
@@ -532,11 +546,11 @@ __global__ __launch_bounds__(64 * W, 1) void attention_kv4_prompt_kernel(AttendA
                     p0[c2 & 1][w][i] = (_Float16)p;
                     if constexpr (S::kParts == 2) {
                         p1[c2 & 1][w][i] = (_Float16)(p - (float)p0[c2 & 1][w][i]);
-                        sum[w] = __builtin_fmaf(p, share[t], sum[w]);
+                        sum[w] += p;
                     }
                 }
                 if constexpr (S::kParts == 1) {  // the sum of what is multiplied: of the rounded probabilities
-                    const _Float16 one = (_Float16)share[t];
+                    const _Float16 one = (_Float16)1.0f;
                     sum[w] = __builtin_amdgcn_fdot2((f16x2){p0[c2 & 1][w][e], p0[c2 & 1][w][e + 1]}, (f16x2){one, one},
                                                     sum[w], false);
                 }
@@ -571,9 +585,6 @@ __global__ __launch_bounds__(64 * W, 1) void attention_kv4_prompt_kernel(AttendA
             behind_values();
             l[0] += sum[0];
             l[1] += sum[1];
-            if (odd)
-#pragma unroll
-                for (int t = 0; t < kPass; ++t) share[t] = 1.0f;
         };
         auto multiply = [&](int step) __attribute__((always_inline)) {
             if constexpr (kSub == kPass) {

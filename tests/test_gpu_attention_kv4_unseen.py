@@ -6,12 +6,9 @@ import numpy as np
 import pytest
 
 import kv_reference as R
-from test_gpu_attention_kv4 import KINDS, Setup
+from test_gpu_attention_kv4 import BOTH, KINDS, Setup
 
 pytestmark = pytest.mark.gpu
-
-# max_added of the kernel of few rows
-KERNELS = [1]
 
 
 def put(s, half, position, x):
@@ -43,7 +40,7 @@ def within(s, q, got, kind, window=0):
 
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("dim,group", [(64, 2), (128, 1), (128, 4), (256, 1)])
-@pytest.mark.parametrize("most", KERNELS)
+@pytest.mark.parametrize("most", BOTH)
 @pytest.mark.parametrize("size", [1e2, 1e5])
 def test_a_large_value_reaches_those_who_see_it(hip, torch_gpu, kind, dim, group, most, size):
     """Values around 1e-3 (scales around 2^-12) and one token's of `size`: rows before it are as exact as without it,
@@ -62,8 +59,22 @@ def test_a_large_value_reaches_those_who_see_it(hip, torch_gpu, kind, dim, group
         s.v[0][token], s.vs[0][token], s.cache.bytes = saved
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("most", BOTH)
+def test_a_large_key_reaches_those_who_see_it(hip, torch_gpu, kind, dim, most):
+    """Keys around 1e-4, whose scales are below the normal numbers of fp16, and one token's of 1e5."""
+    s = Setup(torch_gpu, [50], 1, dim, 16, seed=dim, k_size=1e-4)
+    q = queries(torch_gpu, s, 50, 1, kind, 3e4)
+    for token in (15, 31, 32):
+        saved = s.k[0][token].copy(), s.ks[0][token].copy(), s.cache.bytes.copy()
+        put(s, 0, token, 1e5 * np.linspace(0.5, 1, dim)[None] * (1 - 2 * (np.arange(dim) % 2)))
+        within(s, q, attend(hip, s, q, 50, kind, most), kind)
+        s.k[0][token], s.ks[0][token], s.cache.bytes = saved
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("most", KERNELS)
+@pytest.mark.parametrize("most", BOTH)
 @pytest.mark.parametrize("window", [9, 40])
 def test_a_large_value_before_the_window(hip, torch_gpu, kind, most, window):
     """Rows whose window has left the large token behind, beside rows that still see it."""
