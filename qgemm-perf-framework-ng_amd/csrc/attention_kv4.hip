@@ -597,7 +597,9 @@ hipError_t launch_dim(const AttendArgs &a, const AttendPlan &plan, int type, hip
 // mean over 496 sizes; 38 % at worst, where 7 us are left on the table for one launch instead of two).
 struct Sizes {
     int type, q_heads, kv_heads, head_dim, cus;
-    int64_t requests, max_added, max_length;
+    int64_t requests, max_added, max_length;  // of the requests that the launch is for
+    int64_t launched;                         // all requests times key heads: each has workgroups, if only to find no rows
+    int64_t joined;                           // rows of all: parts are joined by 16 threads each
     bool causal;
 };
 struct Planned {
@@ -618,8 +620,8 @@ Shape shape_of(const Sizes &z, int64_t tile_rows, int64_t keys) {
     const int64_t rows = z.max_added * (z.q_heads / z.kv_heads), heads = std::max<int64_t>(1, z.requests * z.kv_heads);
     const int64_t tiles = std::max<int64_t>(1, (rows + tile_rows - 1) / tile_rows);
     Shape s;
-    // a workgroup takes every tiles-th tile: fewer where the grid would pass 2^31
-    s.tiles = (int)std::min<int64_t>(tiles, std::max<int64_t>(1, (int64_t(1) << 22) / heads));
+    // a workgroup takes every tiles-th tile: fewer where the grid would pass 2^22 workgroups
+    s.tiles = (int)std::min<int64_t>(tiles, std::max<int64_t>(1, (int64_t(1) << 22) / std::max<int64_t>(1, z.launched)));
     s.steps = std::max<int64_t>(1, (z.max_length + keys - 1) / keys);
     s.groups = (double)heads * tiles;
     // of the first and the last row tile, half and half
@@ -627,6 +629,11 @@ Shape shape_of(const Sizes &z, int64_t tile_rows, int64_t keys) {
         std::max<int64_t>(0, std::min(z.max_added, z.max_length) - tile_rows * z.kv_heads / z.q_heads) / 2;
     s.average = (double)std::max<int64_t>(1, ((z.causal ? z.max_length - hidden : z.max_length) + keys - 1) / keys);
     return s;
+}
+
+// HIP takes fewer than 2^32 threads in a launch. (One part of 4 waves always fits: launched is below 2^24.)
+bool fits(const Sizes &z, const Shape &s, int64_t parts, int threads) {
+    return z.launched * s.tiles * parts * threads < int64_t(1) << 32 && (parts == 1 || z.joined < int64_t(1) << 27);
 }
 
 // The parts that a row tile has on average, where the longest has n of `per` steps.
@@ -647,7 +654,7 @@ Planned plan_prompt(const Sizes &z) {
     const double step = z.type == 1 ? 1720 : z.head_dim == 64 ? 3350 : z.head_dim == 128 ? 3750 : 2950, start = 8600;
     Planned best;
     for (const int64_t n : kParts) {
-        if (n > s.steps) break;
+        if (n > s.steps || !fits(z, s, n, 2 * (int)tile_rows)) break;
         const int64_t per = (s.steps + n - 1) / n;
         const double parts = parts_of(s.average, n, per), rounds = s.groups * parts / z.cus;
         double ns = start + per * step;
@@ -672,7 +679,6 @@ Planned plan_prompt(const Sizes &z) {
 // requests of up to 8192 keys, 32 heads over 8 of 128: 66, 59, 55, 46, 52 and 51 us in 1, 2, 3, 4, 5 and 8 parts).
 Planned plan_rows(const Sizes &z) {
     const Shape s = shape_of(z, kRows, kStep);
-    const int64_t groups = std::max<int64_t>(1, z.requests * s.tiles * z.kv_heads);
     const bool two = z.type != 1;
     const double alone = (700 + 4.5 * z.head_dim) * (two ? 1.4 : 1.0), busy = z.head_dim * (two ? 1.9 : 1.4);
     const double start = 3500 + 15 * z.head_dim;
@@ -680,11 +686,11 @@ Planned plan_rows(const Sizes &z) {
     double least = INFINITY;
     Planned best;
     for (const int64_t n : kParts) {
-        if (n > 1 && s.steps < 4 * n) break;
+        if (n > 1 && (s.steps < 4 * n || !fits(z, s, n, 256))) break;
         const int64_t per = (s.steps + n - 1) / n;
         for (const int waves : {4, 8}) {
             const int beside = std::max(1, row_waves(z.head_dim, z.type == 0) / waves);  // workgroups of a CU
-            if (waves == 8 && groups * n > z.cus * beside) break;
+            if (waves == 8 && (s.groups * n > z.cus * beside || !fits(z, s, n, 512))) break;
             auto time = [&](double average) {
                 const double parts = parts_of(average, n, per), rounds = s.groups * parts / z.cus / beside;
                 const double shared = std::min<double>(beside, std::max(1.0, rounds * beside));
@@ -703,7 +709,7 @@ Planned plan_rows(const Sizes &z) {
                 best.plan.parts = (int)((s.steps + per - 1) / per), best.plan.per = (int)per;
             }
         }
-        if (groups * n > 32 * z.cus) break;
+        if (s.groups * n > 32 * z.cus) break;
     }
     return best;
 }
@@ -712,7 +718,7 @@ Planned plan_rows(const Sizes &z) {
 
 AttendPlan plan_attention(int type, int64_t tokens, int64_t requests, int q_heads, int kv_heads, int head_dim,
                           int64_t max_added, int64_t max_length, bool causal, int cus) {
-    Sizes z{type, q_heads, kv_heads, head_dim, cus, requests, max_added, max_length, causal};
+    Sizes z{type, q_heads, kv_heads, head_dim, cus, requests, max_added, max_length, requests * kv_heads, tokens * q_heads, causal};
     AttendPlan p;
     AttendLaunch &main = p.launch[0];
     // A step that serves new prompts and running requests has half of what max_added says, or less: a launch for each, or
