@@ -190,6 +190,10 @@ int pfng_hip_compute_noalloc(int type, const float *activation, const void *weig
  * cache is skipped, a length past the table is cut, and a result that depends on
  * none of them is not touched.
  *
+ * One call is one launch of fewer than 2^32 threads: norms, stores and reads of 2^35
+ * elements and more (of q and k together, or of k), and attention of 2^24 requests
+ * times key heads, are refused.
+ *
  * Element types of keys, values, queries and results; rows of a token's heads are
  * contiguous, tokens `stride` elements apart, both 16-byte aligned. */
 typedef enum { PFNG_F32 = 0, PFNG_BF16 = 1, PFNG_F16 = 2 } pfng_element_type;

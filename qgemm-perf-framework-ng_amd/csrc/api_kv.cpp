@@ -23,8 +23,10 @@ typedef long long ll;
 // Counts above this are refused: positions, keys and slots are 32-bit numbers,
 // and sums of two of them stay so.
 constexpr int64_t kMost = int64_t(1) << 30;
-// Head rows of one call: at 8 rows a workgroup the grid stays below 2^31.
+// Queries' head rows of an attention call, whose workgroups take several row tiles where there are many.
 constexpr int64_t kMostRows = int64_t(1) << 32;
+// HIP takes fewer than 2^32 threads in a launch: workgroups of 256.
+constexpr int64_t kMostGroups = (int64_t(1) << 24) - 1;
 
 int elem_bytes(int type) { return type == PFNG_F32 ? 4 : 2; }
 
@@ -64,6 +66,16 @@ int check_rows(const char *what, const char *name, const void *p, int64_t stride
     return PFNG_OK;
 }
 
+// The kernels that take a row of head_dim elements by head_dim / 8 threads, 2048 elements a workgroup: its workgroups
+// where each takes rows of all heads (heads = 1), or of one head.
+int check_groups(const char *what, int64_t rows, int64_t heads, int head_dim) {
+    const int64_t each = 2048 / head_dim;
+    if ((rows + each - 1) / each > kMostGroups / heads)
+        return fail(PFNG_ERR_INVALID_ARGUMENT, "%s: %lld rows of %d elements are too many for one launch", what,
+                    (ll)(rows * heads), head_dim);
+    return PFNG_OK;
+}
+
 int current_cus(int *cus) {
     int dev = 0;
     if (hipGetDevice(&dev) != hipSuccess) return fail(PFNG_ERR_HIP, "hipGetDevice failed");
@@ -91,7 +103,7 @@ int check_attention(int64_t tokens, int64_t requests, int q_heads, int kv_heads,
     if (kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || q_heads > 65536)
         return fail(PFNG_ERR_INVALID_ARGUMENT, "attention_kv4: q_heads=%d must be a positive multiple of kv_heads=%d",
                     q_heads, kv_heads);
-    if (tokens * q_heads > kMostRows || requests * kv_heads > kMost)
+    if (tokens * q_heads > kMostRows || requests * kv_heads > kMostGroups)
         return fail(PFNG_ERR_INVALID_ARGUMENT, "attention_kv4: tokens=%lld requests=%lld heads=%d are too many", (ll)tokens,
                     (ll)requests, q_heads);
     if (tokens * (q_heads / kv_heads) > kMost)
@@ -158,8 +170,8 @@ int pfng_hip_qk_norm_rope(const void *q, int64_t q_stride, const void *k, int64_
                     rot_dim, head_dim);
     if (!(eps >= 0.0f) || !std::isfinite(eps)) return fail(PFNG_ERR_INVALID_ARGUMENT, "%s: eps must be finite and not negative", what);
     const int64_t rows = tokens * (int64_t(q_heads) + kv_heads);
-    if (rows > kMostRows) return fail(PFNG_ERR_INVALID_ARGUMENT, "%s: %lld rows are too many", what, (ll)rows);
     if (rows == 0) return PFNG_OK;
+    if ((rc = check_groups(what, rows, 1, head_dim))) return rc;
     if (q_heads && ((rc = check_rows(what, "q", q, q_stride, q_heads, head_dim, in_type)) ||
                     (rc = check_rows(what, "q_out", q_out, q_out_stride, q_heads, head_dim, out_type))))
         return rc;
@@ -186,9 +198,9 @@ int pfng_hip_kv4_store(const void *k, int64_t k_stride, const void *v, int64_t v
     const char *what = "kv4_store";
     int rc = check_type(what, type);
     if (rc || (rc = check_cache(what, pages, kv_heads, head_dim, page_size))) return rc;
-    if (tokens < 0 || tokens > kMost || tokens * kv_heads > kMostRows)
-        return fail(PFNG_ERR_INVALID_ARGUMENT, "%s: tokens=%lld", what, (ll)tokens);
+    if (tokens < 0 || tokens > kMost) return fail(PFNG_ERR_INVALID_ARGUMENT, "%s: tokens=%lld", what, (ll)tokens);
     if (tokens == 0) return PFNG_OK;
+    if ((rc = check_groups(what, tokens, kv_heads, head_dim))) return rc;
     if ((rc = check_rows(what, "k", k, k_stride, kv_heads, head_dim, type)) ||
         (rc = check_rows(what, "v", v, v_stride, kv_heads, head_dim, type)))
         return rc;
@@ -207,9 +219,9 @@ int pfng_hip_kv4_read(const void *cache, int64_t pages, int kv_heads, int head_d
     const char *what = "kv4_read";
     int rc = check_type(what, type);
     if (rc || (rc = check_cache(what, pages, kv_heads, head_dim, page_size))) return rc;
-    if (tokens < 0 || tokens > kMost || tokens * kv_heads > kMostRows)
-        return fail(PFNG_ERR_INVALID_ARGUMENT, "%s: tokens=%lld", what, (ll)tokens);
+    if (tokens < 0 || tokens > kMost) return fail(PFNG_ERR_INVALID_ARGUMENT, "%s: tokens=%lld", what, (ll)tokens);
     if (tokens == 0) return PFNG_OK;
+    if ((rc = check_groups(what, tokens, kv_heads, head_dim))) return rc;
     if (!slots || !cache || !k || !v) return fail(PFNG_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
     if (!aligned(slots, 4) || !aligned(cache, 16) || !aligned(k, 16) || !aligned(v, 16))
         return fail(PFNG_ERR_INVALID_ARGUMENT, "%s: the cache, k and v must be 16-byte, slots 4-byte aligned", what);
