@@ -259,7 +259,9 @@ __global__ __launch_bounds__(64 * kWaves, row_waves(D, sizeof(T) == 4) / kWaves)
             mag = rows_max(mag);
             const int exponent = mag > 0.0f && mag < INFINITY ? max(-100, ilogbf(mag)) : 0;
             const float factor = ldexpf(1.0f, 14 - exponent);
+            // (past the largest number only with bf16 queries of 1e36 and more, whose scores any factor tells apart)
             to_log2 = ldexpf(a.scale_log2, exponent - 14 + (kP == 1 ? 24 : 0));
+            to_log2 = fminf(fmaxf(to_log2, -0x1.fffffep127f), 0x1.fffffep127f);
             #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 float sum = 0.0f;

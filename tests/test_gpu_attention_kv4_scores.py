@@ -54,3 +54,28 @@ def test_scores_past_the_units_of_fp32(hip, torch_gpu, kind, dim, most, alike):
                 only = seen[order[-1]]
                 # the result's rounding, and for bf16 those of a probability and of a value to fp16
                 assert (np.abs(got[i, 0] - only) <= R.rounding(only, kind) + 2.0 ** -11 * np.abs(only) + 1e-6).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("most", BOTH)
+def test_queries_up_to_the_end_of_fp32(hip, torch_gpu, kind, dim, most):
+    """Queries of 1e34 to 3e38 with keys of 1e-6: scores that fp32 holds, and the largest of which takes all."""
+    torch = torch_gpu
+    s = Setup(torch, [40], 1, dim, 16, seed=dim, k_size=1e-6)
+    cache, table, lengths = s.device()
+    starts = torch.tensor([0, 40], dtype=torch.int32, device="cuda")
+    for size in (1e34, 1e36, 1e37, 1e38, 3e38):
+        q = size * np.random.default_rng(3).uniform(-1, 1, (40, 1, dim))
+        q = torch.from_numpy(q.astype(np.float32)).cuda().to(getattr(torch, KINDS[kind]))
+        print(f"scores: dim={dim} {kind} max_added={most} size={size}", flush=True)
+        got = hip.attention_kv4(q, cache, table, lengths, starts, max_added=most).double().cpu().numpy()
+        assert np.isfinite(got).all()
+        x = q.double().cpu().numpy()
+        for i in range(40):
+            scores = dim ** -0.5 * (s.k[0][:i + 1, 0] @ x[i, 0])
+            order = np.argsort(scores)
+            reach = dim ** -0.5 * (np.abs(x[i, 0]) @ (8 * np.repeat(np.abs(s.ks[0][:i + 1, 0]), 32, -1)).T).max()
+            if i == 0 or scores[order[-1]] - scores[order[-2]] > reach * 2.0 ** -9:
+                only = s.v[0][order[-1], 0]
+                assert (np.abs(got[i, 0] - only) <= R.rounding(only, kind) + 2.0 ** -11 * np.abs(only) + 1e-6).all()
