@@ -247,7 +247,9 @@ int pfng_hip_kv4_read(const void *cache, int64_t pages, int kv_heads, int head_d
                       const int32_t *slots, int64_t tokens, void *k, void *v, int type, void *stream);
 
 /* Bytes of workspace pfng_hip_attention_kv4 needs for these sizes on the current
- * device (0 where the keys are not split); -1 for sizes that it refuses. */
+ * device (0 where the keys are not split); -1 for sizes that it refuses. The need
+ * goes by how the keys are split and does not grow with the sizes (a batch may need
+ * none where one request of it needs some): ask for the sizes of each call. */
 int64_t pfng_hip_attention_kv4_workspace_size(int type, int64_t tokens, int64_t requests, int q_heads, int kv_heads,
                                               int head_dim, int causal, int64_t max_added, int64_t max_length);
 
@@ -261,10 +263,18 @@ int64_t pfng_hip_attention_kv4_workspace_size(int type, int64_t tokens, int64_t 
  * and a query that sees none gets zeros. causal 0 is cross attention to states of
  * any length. max_added and max_length say how many tokens one request adds and
  * how many keys it has at most: they choose the launch's shape, and larger counts
- * are still computed, only slower. Results of tokens of no request are undefined.
- * A NaN or an infinity in the cache reaches the queries that see it and no others.
- * bf16: keys, values and probabilities enter the products rounded to fp16 (11
- * bits); fp32 and fp16: exact keys and values, probabilities to 22 bits. */
+ * are still computed, only slower, as they are where both say much more than there
+ * is. The window does not go into that choice: where it is far shorter than the
+ * requests, a max_length of window + max_added (in the workspace's query too) says
+ * it. Results of tokens of no request are undefined.
+ * A NaN or an infinity in the cache reaches the queries that see it and no others,
+ * and so does the size of any value: a row's accuracy goes by what it sees.
+ * Maxima, sums and results are in fp32, rounded once. Into the products go
+ *   bf16: probabilities rounded to fp16 (11 bits); with many new tokens keys, values
+ *     and the queries times the scale too;
+ *   fp32 and fp16: exact keys and values, probabilities and fp32 queries to 22 bits.
+ * What a key gives to a result is kept to 2^-34 of the largest value that the row
+ * sees. */
 int pfng_hip_attention_kv4(const void *q, int64_t q_stride, void *out, int64_t out_stride, int type,
                            const int32_t *starts, const int32_t *lengths, int64_t requests, int64_t tokens,
                            int q_heads, const int32_t *block_table, int64_t table_stride, int max_pages,

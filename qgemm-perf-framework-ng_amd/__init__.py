@@ -369,7 +369,8 @@ def block_isums(qtype: int, weight, act_q, m: int, n: int, k: int, stream=None):
 # ---------------------------------------------------------------------------
 
 # As for the products, a small call's time is this binding's own: a tensor that fits passes its checks in one
-# expression, and what does not fit is told apart only then.
+# expression, and what does not fit is told apart only then. Nothing here takes part in autograd: results have no
+# gradient, whatever the inputs.
 
 # pfng_element_type
 F32, BF16, F16 = 0, 1, 2
@@ -579,7 +580,8 @@ def kv4_read(cache, slots, head_dim: int, dtype=None, stream=None):
 
 def attention_kv4_workspace(dtype, tokens: int, requests: int, q_heads: int, kv_heads: int, head_dim: int,
                             max_added: int, max_length: int, causal: bool = True) -> int:
-    """Bytes of workspace attention_kv4 needs for queries of dtype and these sizes on the current device."""
+    """Bytes of workspace attention_kv4 needs for queries of dtype and these sizes on the current device. They do not
+    grow with the sizes (it goes by how the keys are split): ask for the sizes of each call."""
     size = lib().pfng_hip_attention_kv4_workspace_size(_element_type(dtype, "dtype"), tokens, requests, q_heads, kv_heads,
                                                        head_dim, causal, max_added, max_length)
     if size < 0:
@@ -595,7 +597,8 @@ def attention_kv4(q, cache, block_table, lengths, starts=None, max_added: int = 
     of them (starts None: one token each). A query sees the keys up to its own position (causal False: all of the
     request's) and, with a window, only the last `window` of them; one that sees none gets zeros. max_added and
     max_length, the most tokens and keys of one request, choose the launch; the default max_length is what the table
-    holds. scale: head_dim ** -0.5 by default."""
+    holds. With a window far shorter than the requests a max_length of window + max_added chooses a faster one.
+    scale: head_dim ** -0.5 by default."""
     tokens, q_heads, dim = _three(q, "q")
     kind = _element_type(q.dtype, "q")
     pages, kv_heads, page_size = _cache_shape(cache, dim)

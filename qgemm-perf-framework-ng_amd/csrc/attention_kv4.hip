@@ -21,18 +21,22 @@
 //     its leading bit were 2^-14, so that the sum of 32 is 7e-7 of its largest term
 //     off (measured), against 1.5e-8 with q - 8: hence not for fp32 and fp16.
 //   values: q - 8 is exact in fp16, and P times the block's scale is rounded to
-//     fp16 once (bf16 results), or kept as a sum of two fp16 numbers, 22 bits
-//     (fp32 and fp16 results, two products).
+//     fp16 once (bf16 results, which have 8 bits: it moves the error against 64 bits
+//     from 0.0016 to 0.0017), or kept as a sum of two fp16 numbers, 22 bits (fp32 and
+//     fp16 results, two products). These products are scaled by the largest value
+//     scale that the row has seen: a key's share of a result is kept to 2^-34 of the
+//     largest value that the row sees.
 // Queries are scaled by a power of two to below 2^15; fp32 queries are the sum of
 // two fp16 numbers, 22 bits.
 //
 // Few rows read every key once: bound by HBM and by the unpacking beside it. The
 // cache goes to LDS by direct loads, a ring of steps for each wave, so that no
 // register holds what is on its way, and waves share nothing until their sums are
-// joined. 37 requests of up to 8192 keys, 32 heads over 8 of 128, bf16: 43.6 us,
-// 4.1 TB/s, with the vector units busy for 60 % of it; 32767 keys of 32 heads, fp32:
-// 40.8 us, 3.7 TB/s (two products for each of bf16's). One request of 1000 keys:
-// 12.4 us, a chain of launch, lengths, table, keys and sums in one workgroup a head.
+// joined. 37 requests of up to 8192 keys, 32 heads over 8 of 128, bf16: 45.9 us, 179
+// MB at 3.9 TB/s, with the vector units busy for 61 % of it; 32767 keys of 32 heads,
+// fp32: 42.2 us, 3.6 TB/s, 73 % (two products for each of bf16's). (The last-level
+// cache holds some of these caches from call to call.) One request of 1000 keys: 12.6
+// us, a chain of launch, lengths, table, keys and sums in one workgroup a head.
 // Prompts of a few hundred tokens run here too, where the kernel of
 // attention_kv4_prompt.hip would leave most of the chip without a workgroup.
 #include <algorithm>
@@ -594,9 +598,10 @@ hipError_t launch_dim(const AttendArgs &a, const AttendPlan &plan, int type, hip
 }
 
 // The kernel, the parts of the keys and the waves of a workgroup are chosen by models of the kernels' measured times, in ns
-// (one MI355X; both kernels at 840 sizes in 1 to 48 parts: requests 1 to 32 of equal lengths, new tokens 1 to 4096, up to
-// 16384 keys, heads of 64, 128 and 256, fp32 and bf16). What they choose was within 2 % of the fastest choice (geometric
-// mean over 496 sizes; 38 % at worst, where 7 us are left on the table for one launch instead of two).
+// (one MI355X; fitted to both kernels at 840 sizes in 1 to 48 parts: requests 1 to 32 of equal lengths, new tokens 1 to
+// 4096, up to 16384 keys, heads of 64, 128 and 256, fp32 and bf16). With the kernels as they are, what they choose takes
+// 2.5 % longer than the fastest of both kernels, both numbers of waves and 11 of parts (geometric mean over 603 sizes of
+// fp32, bf16 and fp16; 46 % at worst: 16 fp32 tokens of 1016 keys at heads of 256, 22.5 us in one launch, 15.4 in 8 parts).
 struct Sizes {
     int type, q_heads, kv_heads, head_dim, cus;
     int64_t requests, max_added, max_length;  // of the requests that the launch is for
@@ -725,7 +730,7 @@ AttendPlan plan_attention(int type, int64_t tokens, int64_t requests, int q_head
     AttendLaunch &main = p.launch[0];
     // A step that serves new prompts and running requests has half of what max_added says, or less: a launch for each, or
     // running requests' long contexts would go through the prompts' tiles for a row or two (a prompt of 2048 beside 31
-    // requests of up to 8192 keys, 32 heads over 8 of 128, bf16: 404 us in one, 143 in two; 512 beside 63 of 1024: 85, 50).
+    // requests of 8192 keys, 32 heads over 8 of 128, bf16: 404 us in one, 136 in two; 512 beside 63 of 1024: 85, 47).
     const bool mixed = requests > 1 && max_added > kFew && tokens <= requests * max_added / 2;
     Sizes few = z;
     if (mixed) {

@@ -14,24 +14,29 @@
 // 16t + 4g + 0..3 of tile t. Two tiles make the operand of O^T += V^T P^T, whose
 // 32 values are placed in that order: the probabilities stay in their lane.
 //
-// 4096 tokens, 32 heads over 8 of 128, bf16: 157 us (more on cards that clock lower),
-// 875 TFLOP/s; 1024 tokens after 15360 258 us, 1030 TFLOP/s, where a large bf16 product
-// reaches 1212. In the first, the matrix units are busy for 37 % of the cycles, the
-// vector units (exponentials, rounding, unpacking) for 52 %, LDS reads for 27 %; these
+// 4096 tokens, 32 heads over 8 of 128, bf16: 152 to 157 us (more on cards that clock
+// lower), 880 TFLOP/s; 1024 tokens after 15360 280 us, 950 TFLOP/s, where a large bf16
+// product reaches 1212. In the first, the matrix units are busy for 37 % of the cycles,
+// the vector units (exponentials, rounding, unpacking) for 51 %, LDS reads for 27 %; these
 // add up more than they overlap. Decoding tiles beforehand, 64 rows a wave, tiles of
 // twice the keys and other orders of the steps were measured and are no faster.
 // Heads of 64 have half the products for each exponential: 5 prompts of 480 tokens
-// after 1520, 24 heads, 52 us.
+// after 1520, 24 heads, 51 us.
 //
 // Under load this card's clock goes by what it draws: on random numbers the
 // 16x16x32 instruction sustains 2.0 PFLOP/s and 32x32x16 1.68 (its accumulators
 // are read and written twice as often).
 //
-// Decoded values (q - 8) * d are rounded to fp16 once, 11 bits, for bf16 results
-// (products with d below 2^-14 are exact: multiples of 2^-24 below 2^-10). fp32
-// and fp16 results take them exactly, as a sum of two fp16 numbers, and the
-// probabilities and fp32 queries to 22 bits in the same way: three products in
-// the place of one.
+// For bf16 results, which have 8 bits, the operands have fp16's 11: the decoded keys and
+// values (q - 8) * d (products with d below 2^-14 are exact: multiples of 2^-24 below
+// 2^-10), the queries times scale and log2(e), and the probabilities, each rounded once.
+// A score is off by up to 2^-11 of scale * sum |q k| by that, and the error against 64
+// bits at prompts of 480 is 0.00174, where rounding the result alone makes 0.00166.
+// fp32 and fp16 results take keys and values exactly, as a sum of two fp16 numbers, and
+// the probabilities and fp32 queries to 22 bits in the same way: three products in the
+// place of one (two for the scores of fp16, whose queries have no second part). Scores are summed from -base in fp32, so rounded at the size of base,
+// for bf16 results; for the others base is taken off behind the sum. Sums of
+// probabilities are in fp32 and, for bf16 results, of the rounded ones.
 //
 // Scales of 2^13 and more (values past 65504) would overflow: a token with one is
 // decoded divided by 8, and alone (small scales would lose bits, and rows that do
@@ -213,10 +218,10 @@ __global__ __launch_bounds__(64 * W, 1) void attention_kv4_prompt_kernel(AttendA
             first_n[r] = row_first(a, rq, i_row[r]);
         }
 
-        // bf16: the row's query times the scale and log2(e), so that a product is an exponent. fp16 holds that as it is
-        // where the largest element is from 2^-6 to below 2^14 (what is lost below 2^-25 is 2^-19 of that element or
-        // less). Other rows, and those of fp32 and fp16 queries, which keep their bits, are brought to 2^10 by a power
-        // of two, and the products are multiplied by `back`.
+        // bf16: the row's query times the scale and log2(e), rounded to fp16's 11 bits, so that a product is an exponent.
+        // fp16's range takes it where the largest element is from 2^-6 to below 2^14 (what is lost below 2^-25 is 2^-19
+        // of that element or less). Other rows are brought to 2^10 by a power of two, and the products are multiplied by
+        // `back`; so are those of fp32 and fp16 queries, without the scale, so that they keep their bits.
         constexpr bool kRaw = S::kExact;
         f16x8 q[S::kQ][2][NB];
         float back[2] = {1.0f, 1.0f};

@@ -124,7 +124,7 @@ __global__ __launch_bounds__(kTablesThreads) void kv_block_tables_kernel(KvTable
 // HBM-bound. Eight elements a lane: D / 8 lanes a row, four a block, and a
 // workgroup takes 2048 / D neighbouring tokens of one head, keys and values (both
 // by one thread: 15.2 -> 13.0 us). 2048 tokens of 32 heads of 128: stored from bf16
-// in 12.3 us, 3.5 TB/s, read to fp32 in 17.7, 4.3 TB/s.
+// in 13.1 us, 3.3 TB/s, read to fp32 in 17.7, 4.3 TB/s.
 constexpr int kRowThreads = 256;
 
 template <int D>
